@@ -119,6 +119,14 @@ __device__ __forceinline__ int chunk_at(int row, int c) {
     return row * (DT / 8) + (c ^ swizzle<DT>(row));
 }
 
+// A product as its 32-bit value.  fp16 has an instruction that multiplies and rounds to
+// 16 bits at once; with it in one of two places, the value that is stored and the one that
+// is taken off to see what its rounding left out differ by a whole step now and then.
+__device__ __forceinline__ float formed(float v) {
+    asm("" : "+v"(v));
+    return v;
+}
+
 // N values times f to o, what their rounding leaves out to o_low (or null).
 template <typename T, int N>
 __device__ __forceinline__ void put_rounded(char* o, char* o_low, int64_t at, const float (&v)[N],
@@ -127,7 +135,7 @@ __device__ __forceinline__ void put_rounded(char* o, char* o_low, int64_t at, co
     vec high, low;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-        const float x = v[i] * f;
+        const float x = formed(v[i] * f);
         high[i] = (typename T::elem)x;
         low[i] = (typename T::elem)(x - (float)high[i]);
     }
@@ -194,7 +202,7 @@ __device__ __forceinline__ typename T::vec8 pack(const f32x16& p, int b) {
     return out;
 }
 
-// What that rounding left out, rounded in its turn.
+// What that rounding left out, rounded in its turn; p is `formed`.
 template <typename T>
 __device__ __forceinline__ typename T::vec8 pack_low(const f32x16& p, int b) {
     typename T::vec8 out;

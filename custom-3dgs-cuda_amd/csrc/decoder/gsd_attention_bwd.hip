@@ -333,6 +333,7 @@ __global__ __launch_bounds__(kThreads, 2) void dq_kernel(GradArgs g) {
             for (int i = 0; i < 16; ++i) {
                 const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], a.scale_log2, off));
                 s[i] = p * (dp[i] * ds_scale);
+                if constexpr (kFew) s[i] = formed(s[i]);
             }
             if (left < kTile) {
                 const int me = opaque(lane);
@@ -474,6 +475,7 @@ __global__ __launch_bounds__(kThreads, kFew ? 2 : 3) void dkdv_kernel(GradArgs g
                             const int j = 4 * i4 + i;
                             s[h][j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[h][j], a.scale_log2, of[i]));
                             dp[h][j] = s[h][j] * (dp[h][j] * ds_scale);
+                            if constexpr (kFew) dp[h][j] = formed(dp[h][j]);
                         }
                     }
                 };
@@ -634,6 +636,7 @@ __global__ __launch_bounds__(kThreads, 2) void dkdv_pair_kernel(GradArgs g) {
                         const int j = 4 * i4 + i;
                         s[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j], a.scale_log2, of[i]));
                         dp[j] = s[j] * (dp[j] * ds_scale);
+                        if constexpr (kFew) dp[j] = formed(dp[j]);
                     }
                 }
                 vec8 keep[2], keep_low[2];
