@@ -48,8 +48,8 @@ struct F16 {
     // p, and the factor taken out of the sums.  The forward's p = 2^(s - m) is at
     // most 2^kSlack; with 2^7 it stays below 2^15 as well.
     static constexpr float kShift = 7.0f, kGradShift = 15.0f;
-    // ds = p (dp - delta) is of do's size: it is scaled by a power of two
-    // that brings do's largest value to [1, 2)
+    // ds = p (dp - delta) has the size of do times v: it is scaled by a power of two
+    // from their norms, a row's for dq and a key's for dk
     static constexpr bool kScaled = true;
     static __device__ __forceinline__ f32x16 mma(vec8 a, vec8 b, f32x16 c) {
         return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);

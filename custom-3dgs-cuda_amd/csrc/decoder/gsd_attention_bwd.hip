@@ -42,8 +42,10 @@ struct GradArgs {
     int64_t dob, dol, doh;  // bytes
     // [batch kv_heads, 2, rows]: shift - lse (-infinity for a row without a key), -delta
     float* stat;
-    float* top;  // max |do| per delta block
-    int32_t top_blocks;
+    // fp16: [batch kv_heads, 2, top_blocks], max |do| (a row's norm) and max |delta| per
+    // block of rows, and [batch kv_heads, value_blocks], max |v| per block of keys
+    float *top, *value_top;
+    int32_t top_blocks, value_blocks;
     char *dq, *dk, *dv;
     float *partial_dq, *partial_dk, *partial_dv;
 };
@@ -76,17 +78,57 @@ __device__ __forceinline__ void zero_keys(const GradArgs& g, uint32_t group) {
     store_any(g.dv + 16 * id, u32x4{0, 0, 0, 0});
 }
 
+// The maximum over a work-group, in its first thread.
+__device__ __forceinline__ float group_max(float v, float (&part)[kWaves]) {
+    v = wave_max(v);
+    if (lane_id() == 0) part[threadIdx.x / kWave] = v;
+    __syncthreads();
+    return fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
+}
+
+// max |v| over 64 keys that take part, 16 lanes per key.
+template <typename T>
+__device__ __forceinline__ void value_norms(const GradArgs& g, uint32_t group,
+                                            float (&part)[kWaves]) {
+    const AttnArgs& a = g.f;
+    const int bh = (int)(group / g.value_blocks), block = (int)(group % g.value_blocks);
+    const int b = bh / a.kv_heads, kvh = bh % a.kv_heads;
+    const int c = threadIdx.x % 16;
+    float top = 0.0f;
+#pragma unroll
+    for (int j = 0; j < kDeltaRows / 16; ++j) {
+        const int64_t key = (int64_t)block * kDeltaRows + j * 16 + (int)threadIdx.x / 16;
+        float square = 0.0f;
+        if (8 * c < a.dim && key_valid(a, b, key)) {
+            const auto x = load_any<typename T::vec8>(a.v + b * a.vb + key * a.vs + kvh * a.vh + 16 * c);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) square = __builtin_fmaf((float)x[i], (float)x[i], square);
+        }
+#pragma unroll
+        for (int d = 8; d > 0; d >>= 1) square += __shfl_xor(square, d);
+        top = fmaxf(top, square);
+    }
+    top = group_max(top, part);
+    if (threadIdx.x == 0) g.value_top[group] = sqrtf(top);
+}
+
 // ---- delta: 16 lanes per row of up to 128 elements ----
-// The work-groups behind those of the rows write the zeros of keys that take no part:
-// 2 x 1237 x 8260, 8 heads of 128, takes 390 us with lengths, forward and backward, 396
-// with a launch for the zeros, and 2 x 32 x 300, which the host bounds, 86 and 89.
+// The work-groups behind those of the rows find the largest |v| (fp16) and write the
+// zeros of keys that take no part: 2 x 1237 x 8260, 8 heads of 128, takes 390 us with
+// lengths, forward and backward, 396 with a launch for the zeros, and 2 x 32 x 300, which
+// the host bounds, 86 and 89.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void delta_kernel(GradArgs g) {
     const AttnArgs& a = g.f;
-    __shared__ float s_top[kThreads / kWave];
-    const uint32_t groups = (uint32_t)a.batch * a.kv_heads * g.top_blocks;
+    __shared__ float s_top[kWaves], s_delta[kWaves];
+    const uint32_t heads = (uint32_t)a.batch * a.kv_heads;
+    uint32_t groups = heads * g.top_blocks;
     if (blockIdx.x >= groups) {
-        zero_keys(g, blockIdx.x - groups);
+        const uint32_t values = T::kScaled ? heads * g.value_blocks : 0;
+        if (blockIdx.x - groups < values)
+            value_norms<T>(g, blockIdx.x - groups, s_top);
+        else
+            zero_keys(g, blockIdx.x - groups - values);
         return;
     }
     const int bh = (int)(blockIdx.x / g.top_blocks);
@@ -94,11 +136,11 @@ __global__ __launch_bounds__(kThreads) void delta_kernel(GradArgs g) {
     const int b = bh / a.kv_heads, kvh = bh % a.kv_heads;
     const int c = threadIdx.x % 16;
     const int64_t queries = a.rows / a.group;
-    float top = 0.0f;
+    float top = 0.0f, top_delta = 0.0f;
 #pragma unroll
     for (int j = 0; j < kDeltaRows / 16; ++j) {
         const int row = block * kDeltaRows + j * 16 + (int)threadIdx.x / 16;
-        float dot = 0.0f;
+        float dot = 0.0f, square = 0.0f;
         if (row < a.rows && 8 * c < a.dim) {
             const RowAt at = row_at(a, kvh, row);
             const auto x = load_any<typename T::vec8>(g.d_o + b * g.dob + at.l * g.dol +
@@ -112,38 +154,74 @@ __global__ __launch_bounds__(kThreads) void delta_kernel(GradArgs g) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 dot = __builtin_fmaf((float)x[i], (float)y[i] + (float)z[i], dot);
-                top = fmaxf(top, fabsf((float)x[i]));
+                if (T::kScaled) square = __builtin_fmaf((float)x[i], (float)x[i], square);
             }
         }
 #pragma unroll
-        for (int d = 8; d > 0; d >>= 1) dot += __shfl_xor(dot, d);
+        for (int d = 8; d > 0; d >>= 1) {
+            dot += __shfl_xor(dot, d);
+            if (T::kScaled) square += __shfl_xor(square, d);
+        }
         if (c == 0 && row < a.rows) {
             const float lse = a.lse[(int64_t)bh * a.rows + row];
             float* const to = g.stat + 2 * (int64_t)bh * a.rows + row;
             to[0] = lse == -__builtin_inff() ? lse : T::kGradShift - lse;
             to[a.rows] = -dot;
         }
+        top = fmaxf(top, square);
+        top_delta = fmaxf(top_delta, fabsf(dot));
     }
     if (!T::kScaled) return;
-    top = wave_max(top);
-    if (lane_id() == 0) s_top[threadIdx.x / kWave] = top;
-    __syncthreads();
-    if (threadIdx.x == 0)
-        g.top[(int64_t)bh * g.top_blocks + block] =
-            fmaxf(fmaxf(s_top[0], s_top[1]), fmaxf(s_top[2], s_top[3]));
+    top = group_max(top, s_top);
+    top_delta = group_max(top_delta, s_delta);
+    if (threadIdx.x == 0) {
+        float* const to = g.top + 2 * (int64_t)bh * g.top_blocks + block;
+        to[0] = sqrtf(top);
+        to[g.top_blocks] = top_delta;
+    }
 }
 
-// The power of two that brings the problem's largest |do| to [1, 2); 1 where
-// there is none, or it is not finite.
-template <typename T>
-__device__ __forceinline__ float grad_scale(const GradArgs& g, int bh) {
-    if (!T::kScaled) return 1.0f;
+// The largest of n, by a wave.
+__device__ __forceinline__ float largest(const float* v, int n) {
     float top = 0.0f;
-    for (int i = lane_id(); i < g.top_blocks; i += kWave)
-        top = fmaxf(top, g.top[(int64_t)bh * g.top_blocks + i]);
-    top = wave_max(top);
-    if (!(top > 0.0f) || top > 3.0e38f) return 1.0f;
-    return __builtin_ldexpf(1.0f, 1 - __builtin_amdgcn_frexp_expf(top));
+    for (int i = lane_id(); i < n; i += kWave) top = fmaxf(top, v[i]);
+    return wave_max(top);
+}
+
+// The power of two that ds is scaled by before it is rounded, from a bound on |dp -
+// delta|: |do| |v| + |delta|, of a row for dq and of a key for dk, which take it out of
+// their sums again.  It brings the bound to [2^14, 2^15), so that ds, p times that with p
+// at most 1, neither overflows fp16 nor loses digits before it is 2^-28 of the bound (p of
+// 1 / 32400 and a bound that is 2^5 too high leave 2^8).  1 where the bound is 0 or not
+// finite.  In what follows a lane holds half of the row's or key's elements in `held`.
+template <typename T, int N>
+__device__ __forceinline__ float held_norm(const typename T::vec8 (&held)[N]) {
+    float square = 0.0f;
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            square = __builtin_fmaf((float)held[j][i], (float)held[j][i], square);
+    return sqrtf(square + other_half(square));
+}
+__device__ __forceinline__ float scale_of(float bound) {
+    if (!(bound > 0.0f) || !(bound < __builtin_inff())) return 1.0f;
+    return __builtin_ldexpf(1.0f, 15 - __builtin_amdgcn_frexp_expf(bound));
+}
+template <typename T, int N>
+__device__ __forceinline__ float row_scale(const GradArgs& g, int bh,
+                                           const typename T::vec8 (&d_o)[N], float delta) {
+    if (!T::kScaled) return 1.0f;
+    const float value = largest(g.value_top + (int64_t)bh * g.value_blocks, g.value_blocks);
+    return scale_of(__builtin_fmaf(held_norm<T>(d_o), value, fabsf(delta)));
+}
+template <typename T, int N>
+__device__ __forceinline__ float key_scale(const GradArgs& g, int bh,
+                                           const typename T::vec8 (&v)[N]) {
+    if (!T::kScaled) return 1.0f;
+    const float* from = g.top + 2 * (int64_t)bh * g.top_blocks;
+    const float d_o = largest(from, g.top_blocks), delta = largest(from + g.top_blocks, g.top_blocks);
+    return scale_of(__builtin_fmaf(d_o, held_norm<T>(v), delta));
 }
 
 // Tiles of kRows of the problem's rows straight to LDS, one after the other, for q
@@ -289,14 +367,15 @@ __global__ __launch_bounds__(kThreads, 2) void dq_kernel(GradArgs g) {
     vec8 q[DC / 16], d_o[DC / 16];
     hold<T, DC>(q, a.q + b * a.qb + at.l * a.ql + at.head * a.qh, live, a.dim);
     hold<T, DC>(d_o, g.d_o + b * g.dob + at.l * g.dol + at.head * g.doh, live, a.dim);
-    const float up = grad_scale<T>(g, bh);
-    const float ds_scale = up * __builtin_ldexpf(1.0f, -(int)T::kGradShift);
     float off = -__builtin_inff(), minus_delta = 0.0f;
     if (live) {
         const float* from = g.stat + 2 * (int64_t)bh * a.rows + row;
         off = from[0];
         minus_delta = from[a.rows];
     }
+    // with the 2^kGradShift that p carries taken out
+    const float ds_scale =
+        row_scale<T>(g, bh, d_o, minus_delta) * __builtin_ldexpf(1.0f, -(int)T::kGradShift);
     f32x16 begin;  // dp's sums begin at -delta, which saves its addition to each
 #pragma unroll
     for (int i = 0; i < 16; ++i) begin[i] = minus_delta;
@@ -367,7 +446,7 @@ __global__ __launch_bounds__(kThreads, 2) void dq_kernel(GradArgs g) {
         }
     }
     if (!live) return;
-    const float f = a.scale / up;
+    const float f = a.scale / (ds_scale * __builtin_ldexpf(1.0f, (int)T::kGradShift));
     if (a.parts == 1) {
         const int64_t queries = a.rows / a.group;
         put<T, DC, false>(dq, f, g.dq + 2 * (((b * queries + at.l) * a.heads + at.head) * (int64_t)a.dim),
@@ -405,8 +484,7 @@ __global__ __launch_bounds__(kThreads, kFew ? 2 : 3) void dkdv_kernel(GradArgs g
     f32x16 dk[DT / 32], dv[DT / 32];
     clear(dk);
     clear(dv);
-    const float up = grad_scale<T>(g, bh);
-    const float ds_scale = up * __builtin_ldexpf(1.0f, -(int)T::kGradShift);
+    float ds_scale = 1.0f;
     int t = (int)part * a.tiles_per_part, end = t + a.tiles_per_part;
     end = end < a.tiles ? end : a.tiles;
 
@@ -435,6 +513,8 @@ __global__ __launch_bounds__(kThreads, kFew ? 2 : 3) void dkdv_kernel(GradArgs g
         vec8 k[DT / 16], v[DT / 16];
         hold<T, DT>(k, a.k + b * a.kb + key * a.ks + kvh * a.kh, valid, a.dim);
         hold<T, DT>(v, a.v + b * a.vb + key * a.vs + kvh * a.vh, valid, a.dim);
+        // with the 2^kGradShift that p carries taken out
+        ds_scale = key_scale<T>(g, bh, v) * __builtin_ldexpf(1.0f, -(int)T::kGradShift);
         dma_wait();
         __syncthreads();
         auto step = [&](const char* tile_q, const char* tile_g, const float* stat, char* next_q,
@@ -520,7 +600,7 @@ __global__ __launch_bounds__(kThreads, kFew ? 2 : 3) void dkdv_kernel(GradArgs g
         }
     }
     if (!valid) return;  // their gradients are written as 0 with delta
-    const float fk = a.scale / up;
+    const float fk = a.scale / (ds_scale * __builtin_ldexpf(1.0f, (int)T::kGradShift));
     const float fv = __builtin_ldexpf(1.0f, -(int)T::kGradShift);
     if (a.parts == 1) {
         const int64_t to = 2 * (((b * a.keys + key) * a.kv_heads + kvh) * (int64_t)a.dim);
@@ -567,8 +647,7 @@ __global__ __launch_bounds__(kThreads, 2) void dkdv_pair_kernel(GradArgs g) {
     const int64_t key = a.list && valid ? a.list[(int64_t)b * a.keys + at_key] : at_key;
     f32x16 acc[DC / 32];
     clear(acc);
-    const float up = grad_scale<T>(g, bh);
-    const float ds_scale = up * __builtin_ldexpf(1.0f, -(int)T::kGradShift);
+    float ds_scale = 1.0f;
     int t = (int)part * a.tiles_per_part, end = t + a.tiles_per_part;
     end = end < a.tiles ? end : a.tiles;
 
@@ -594,6 +673,8 @@ __global__ __launch_bounds__(kThreads, 2) void dkdv_pair_kernel(GradArgs g) {
         vec8 k[DC / 16], v[DC / 16];
         hold<T, DC>(k, a.k + b * a.kb + key * a.ks + kvh * a.kh, valid, a.dim);
         hold<T, DC>(v, a.v + b * a.vb + key * a.vs + kvh * a.vh, valid, a.dim);
+        // with the 2^kGradShift that p carries taken out
+        ds_scale = key_scale<T>(g, bh, v) * __builtin_ldexpf(1.0f, -(int)T::kGradShift);
         dma_wait();
         __syncthreads();
         auto step = [&](const char* tile_q, const char* tile_g, const float* stat, char* next_q,
@@ -695,7 +776,8 @@ __global__ __launch_bounds__(kThreads, 2) void dkdv_pair_kernel(GradArgs g) {
         }
     }
     if (!valid) return;
-    const float f = role ? a.scale / up : __builtin_ldexpf(1.0f, -(int)T::kGradShift);
+    const float f = role ? a.scale / (ds_scale * __builtin_ldexpf(1.0f, (int)T::kGradShift))
+                         : __builtin_ldexpf(1.0f, -(int)T::kGradShift);
     if (a.parts == 1) {
         const int64_t to = 2 * (((b * a.keys + key) * a.kv_heads + kvh) * (int64_t)a.dim);
         put<T, DC, false>(acc, f, (role ? g.dk : g.dv) + to, a.dim);
@@ -777,7 +859,8 @@ hipError_t launch_typed(const GradArgs& base, const AttentionSplit& sq, const At
     const int64_t units = heads * base.f.keys * (base.f.dim / 8);
     const int64_t zero_groups =
         base.dk && (base.f.mask || base.f.lengths) ? (units + kThreads - 1) / kThreads : 0;
-    run(delta_kernel<T>, base, heads * base.top_blocks + zero_groups);
+    const int64_t value_groups = T::kScaled ? heads * base.value_blocks : 0;
+    run(delta_kernel<T>, base, heads * base.top_blocks + value_groups + zero_groups);
     if (base.f.list) {
         const hipError_t e = launch_key_list(base.f, st);
         if (e != hipSuccess) return e;
@@ -852,6 +935,10 @@ int64_t attention_top_blocks(const gsd_attention& g) {
     return (g.queries * (g.heads / g.kv_heads) + kDeltaRows - 1) / kDeltaRows;
 }
 
+int64_t attention_value_blocks(const gsd_attention& g) {
+    return (g.keys + kDeltaRows - 1) / kDeltaRows;
+}
+
 hipError_t launch_attention_backward(const gsd_attention& a, const gsd_attention_grad& gr,
                                      const AttentionSplit& sq, const AttentionSplit& sk,
                                      const AttentionBackwardBuffers& buf, hipStream_t st) {
@@ -864,6 +951,9 @@ hipError_t launch_attention_backward(const gsd_attention& a, const gsd_attention
     g.stat = buf.stat;
     g.top = buf.top;
     g.top_blocks = (int32_t)attention_top_blocks(a);
+    g.value_top = buf.value_top;
+    // dq alone needs the values' norms
+    g.value_blocks = gr.dq ? (int32_t)attention_value_blocks(a) : 0;
     g.dq = static_cast<char*>(gr.dq);
     g.dk = static_cast<char*>(gr.dk);
     g.dv = static_cast<char*>(gr.dv);

@@ -146,7 +146,7 @@ ForwardLayout forward_layout(const gsd_attention& a, const gsd::AttentionSplit& 
 }
 
 struct BackwardLayout {
-    size_t stat, top, dq, dk, dv, list, end;
+    size_t stat, top, value_top, dq, dk, dv, list, end;
 };
 BackwardLayout backward_layout(const gsd_attention& a, const gsd::AttentionSplit& sq,
                                const gsd::AttentionSplit& sk) {
@@ -158,7 +158,9 @@ BackwardLayout backward_layout(const gsd_attention& a, const gsd::AttentionSplit
         return at;
     };
     l.stat = take(8 * rows_of(a));
-    l.top = take(4 * (size_t)a.batch * (size_t)a.kv_heads * (size_t)gsd::attention_top_blocks(a));
+    const size_t tops = a.dtype == GSD_F16 ? 4 * (size_t)a.batch * (size_t)a.kv_heads : 0;
+    l.top = take(2 * tops * (size_t)gsd::attention_top_blocks(a));
+    l.value_top = take(tops * (size_t)gsd::attention_value_blocks(a));
     l.dq = take(sq.parts > 1 ? 4 * (size_t)sq.parts * rows_of(a) * (size_t)a.dim : 0);
     const size_t keys = sk.parts > 1 ? 4 * (size_t)sk.parts * key_rows_of(a) * (size_t)a.dim : 0;
     l.dk = take(keys);
@@ -304,16 +306,18 @@ int gsd_cross_attention_backward(const gsd_attention* a, const gsd_attention_gra
     const gsd::AttentionSplit sq = gsd::attention_split_dq(*a);
     const gsd::AttentionSplit sk = gsd::attention_split_dkdv(*a);
     GSD_REQUIRE(grid_fits(*a, sq) && grid_fits(*a, sk), "too many rows or keys");
-    GSD_REQUIRE((__int128)a->batch * a->kv_heads * gsd::attention_top_blocks(*a) <= kMaxGroups &&
-                    (__int128)a->batch * a->kv_heads * a->keys * a->dim <= 2048 * (__int128)kMaxGroups,
+    // delta's work-groups: of rows, of values, of zeros (2048 values each)
+    GSD_REQUIRE((__int128)a->batch * a->kv_heads *
+                        (gsd::attention_top_blocks(*a) + gsd::attention_value_blocks(*a) +
+                         (__int128)a->keys * a->dim / 2048 + 2) <= kMaxGroups,
                 "too many rows or keys");
     const BackwardLayout l = backward_layout(*a, sq, sk);
     if (ws_bytes < l.end || (l.end && !ws))
         return fail(GSR_ERR_WORKSPACE, "workspace of %zu bytes, %zu needed", ws_bytes, l.end);
     GSD_REQUIRE(aligned(ws, 16), "the workspace must be 16-byte aligned");
     const gsd::AttentionBackwardBuffers buf{at<float>(ws, l.stat), at<float>(ws, l.top),
-                                            at<float>(ws, l.dq), at<float>(ws, l.dk),
-                                            at<float>(ws, l.dv),
+                                            at<float>(ws, l.value_top), at<float>(ws, l.dq),
+                                            at<float>(ws, l.dk), at<float>(ws, l.dv),
                                             a->key_mask ? at<int32_t>(ws, l.list) : nullptr};
     GSD_HIP(gsd::launch_attention_backward(*a, *g, sq, sk, buf, as_stream(stream)),
             "cross_attention_backward");

@@ -38,14 +38,18 @@ hipError_t launch_attention(const gsd_attention& a, const AttentionSplit& sp, fl
                             float* partial_lse, int32_t* list, hipStream_t st);
 
 struct AttentionBackwardBuffers {
-    float* stat;         // [batch kv_heads, rows, 2]
-    float* top;          // max |do| per block of the delta kernel, [batch kv_heads, top_blocks]
+    float* stat;         // [batch kv_heads, 2, rows]
+    // (fp16) the largest |do| and |delta| per block of rows, [batch kv_heads, 2, top_blocks],
+    // and |v| per block of keys, [batch kv_heads, value_blocks]
+    float* top;
+    float* value_top;
     float* partial_dq;   // [parts, batch kv_heads, rows, dim]
     float* partial_dk;   // [parts, batch kv_heads, keys, dim]
     float* partial_dv;
     int32_t* list;       // [batch (keys + 1)] where there is a mask
 };
 int64_t attention_top_blocks(const gsd_attention& a);
+int64_t attention_value_blocks(const gsd_attention& a);
 hipError_t launch_attention_backward(const gsd_attention& a, const gsd_attention_grad& g,
                                      const AttentionSplit& sq, const AttentionSplit& sk,
                                      const AttentionBackwardBuffers& buf, hipStream_t st);
