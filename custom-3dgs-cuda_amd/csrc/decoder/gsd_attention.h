@@ -25,6 +25,9 @@
 
 namespace gsd {
 
+// of a lambda whose captures live in registers
+#define GSD_INLINE __attribute__((always_inline))
+
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
 // The forward's sums are scaled anew only where a row's maximum has grown by
@@ -103,6 +106,14 @@ __device__ __forceinline__ uint32_t work_of(uint32_t id, uint32_t batch_total) {
 // rows' low bits in the chunk's low bits it costs 0.57, and 7 times as much for
 // read_rows without a swizzle.
 constexpr int kTile = 64;
+
+// p and ds are rounded to the type for their products: the errors average out over the
+// sums' terms, to that of the result's own rounding.  Up to this many keys that take part
+// (or rows, in dk and dv) they need not: one query and two keys give 2.5 times a result's
+// own rounding.  What the rounding left out is then multiplied too.  A batch's keys count
+// as its length or mask leaves them, not as they are padded.
+constexpr int kFewTerms = 64;
+static_assert(kFewTerms <= kTile, "so few keys are one tile");
 
 // Heads up to 64 lie in rows of DT = 64, others in rows of 128.  Of those the products
 // take DC elements: 96 where a head has no more, all 128 otherwise.  4096 x 32400, 16

@@ -28,13 +28,11 @@ namespace {
 constexpr int kHeld = 128;  // rows (dq) or keys (dk, dv) that a work-group holds
 constexpr int kDeltaRows = 64;
 
-// p and ds are rounded to the type for their products with do, q and k: their
-// errors average out over the sums' terms, to that of the result's own rounding.
-// With few rows or keys they need not (one query and two keys: 2.5 times a result's
-// own rounding), so what the rounding left out is then multiplied too (kFew), which
-// makes dk and dv of 64 x 32400, 16 heads of 128, 7% and dq 10% longer (199 and 62 us)
-// and 4096 x 64 no longer (21 and 14 us).
-bool few_terms(int64_t rows, int64_t keys) { return rows <= 64 || keys <= 64; }
+// Few terms (kFewTerms) that the sizes show make for kernels of their own (kFew): making up
+// for the roundings makes dk and dv of 64 x 32400, 16 heads of 128, 7% and dq 10% longer
+// (199 and 62 us) and 4096 x 64 no longer (21 and 14 us).  Where only a batch's length or
+// mask shows them, the kernels' work-groups see it and take that path.
+bool few_terms(int64_t rows, int64_t keys) { return rows <= kFewTerms || keys <= kFewTerms; }
 
 struct GradArgs {
     AttnArgs f;
@@ -382,7 +380,9 @@ __global__ __launch_bounds__(kThreads, 2) void dq_kernel(GradArgs g) {
     f32x16 dq[DC / 32];
     clear(dq);
 
-    auto step = [&](const char* tile_k, const char* tile_v, char* next_k, char* next_v) -> bool {
+    auto step = [&](auto low, const char* tile_k, const char* tile_v, char* next_k,
+                    char* next_v) GSD_INLINE -> bool {
+        constexpr bool kLow = decltype(low)::value;
         const int left = walk.left();
         walk.next();
         const bool more = walk.more();
@@ -412,7 +412,7 @@ __global__ __launch_bounds__(kThreads, 2) void dq_kernel(GradArgs g) {
             for (int i = 0; i < 16; ++i) {
                 const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], a.scale_log2, off));
                 s[i] = p * (dp[i] * ds_scale);
-                if constexpr (kFew) s[i] = formed(s[i]);
+                if constexpr (kLow) s[i] = formed(s[i]);
             }
             if (left < kTile) {
                 const int me = opaque(lane);
@@ -427,10 +427,10 @@ __global__ __launch_bounds__(kThreads, 2) void dq_kernel(GradArgs g) {
                 for (int db = 0; db < DC / 32; ++db) {
                     const vec8 kt = read_columns<T, DT>(tile_k, 32 * h + 16 * k, db);
                     dq[db] = T::mma(kt, ds, dq[db]);
-                    if constexpr (kFew) dq[db] = T::mma(kt, pack_low<T>(s, k), dq[db]);
+                    if constexpr (kLow) dq[db] = T::mma(kt, pack_low<T>(s, k), dq[db]);
                 }
             }
-            if constexpr (!kFew) pace<DC / 16, 2, 1, 2>();
+            if constexpr (!kLow) pace<DC / 16, 2, 1, 2>();
             __builtin_amdgcn_sched_barrier(0);
         }
         if (more) {
@@ -442,8 +442,12 @@ __global__ __launch_bounds__(kThreads, 2) void dq_kernel(GradArgs g) {
     if (walk.more()) {
         dma_wait();
         __syncthreads();
-        while (step(s_k0, s_v0, s_k1, s_v1) && step(s_k1, s_v1, s_k0, s_v0)) {
-        }
+        using Low = std::integral_constant<bool, kFew>;
+        if (!kFew && __builtin_expect(walk.n <= kFewTerms, 0))
+            step(std::true_type{}, s_k0, s_v0, s_k1, s_v1);
+        else
+            while (step(Low{}, s_k0, s_v0, s_k1, s_v1) && step(Low{}, s_k1, s_v1, s_k0, s_v0)) {
+            }
     }
     if (!live) return;
     const float f = a.scale / (ds_scale * __builtin_ldexpf(1.0f, (int)T::kGradShift));
@@ -478,7 +482,8 @@ __global__ __launch_bounds__(kThreads, kFew ? 2 : 3) void dkdv_kernel(GradArgs g
 
     // with a mask, the block's keys are the next of the list
     const int at_key = (int)block * kHeld + wave * 32 + (lane & 31);
-    const bool valid = at_key < (a.list ? a.counts[b] : admitted_keys(a, b));
+    const int keys = a.list ? a.counts[b] : admitted_keys(a, b);
+    const bool valid = at_key < keys;
     const bool busy = ballot(valid) != 0;  // else a wave only loads and waits
     const int64_t key = a.list && valid ? a.list[(int64_t)b * a.keys + at_key] : at_key;
     f32x16 dk[DT / 32], dv[DT / 32];
@@ -517,8 +522,9 @@ __global__ __launch_bounds__(kThreads, kFew ? 2 : 3) void dkdv_kernel(GradArgs g
         ds_scale = key_scale<T>(g, bh, v) * __builtin_ldexpf(1.0f, -(int)T::kGradShift);
         dma_wait();
         __syncthreads();
-        auto step = [&](const char* tile_q, const char* tile_g, const float* stat, char* next_q,
-                        char* next_g, float* next_stat) -> bool {
+        auto step = [&](auto low, const char* tile_q, const char* tile_g, const float* stat,
+                        char* next_q, char* next_g, float* next_stat) GSD_INLINE -> bool {
+            constexpr bool kLow = decltype(low)::value;
             const bool more = ++t < end;
             if (more) {
                 rq.next();
@@ -555,7 +561,7 @@ __global__ __launch_bounds__(kThreads, kFew ? 2 : 3) void dkdv_kernel(GradArgs g
                             const int j = 4 * i4 + i;
                             s[h][j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[h][j], a.scale_log2, of[i]));
                             dp[h][j] = s[h][j] * (dp[h][j] * ds_scale);
-                            if constexpr (kFew) dp[h][j] = formed(dp[h][j]);
+                            if constexpr (kLow) dp[h][j] = formed(dp[h][j]);
                         }
                     }
                 };
@@ -569,7 +575,7 @@ __global__ __launch_bounds__(kThreads, kFew ? 2 : 3) void dkdv_kernel(GradArgs g
                             const vec8 qt = read_columns<T, DT>(tile_q, 32 * h + 16 * b2, db);
                             dv[db] = T::mma(gt, p, dv[db]);
                             dk[db] = T::mma(qt, ds, dk[db]);
-                            if constexpr (kFew) {
+                            if constexpr (kLow) {
                                 dv[db] = T::mma(gt, pack_low<T>(s[h], b2), dv[db]);
                                 dk[db] = T::mma(qt, pack_low<T>(dp[h], b2), dk[db]);
                             }
@@ -582,7 +588,7 @@ __global__ __launch_bounds__(kThreads, kFew ? 2 : 3) void dkdv_kernel(GradArgs g
                     scores(h);
                     softmax(h);
                     sums(h);
-                    if constexpr (!kFew) {
+                    if constexpr (!kLow) {
                         pace<kSteps, 2, 2, 3>();
                         pace<kSteps, 4, 2, 2>();
                     }
@@ -595,9 +601,15 @@ __global__ __launch_bounds__(kThreads, kFew ? 2 : 3) void dkdv_kernel(GradArgs g
             }
             return more;
         };
-        while (step(s_q0, s_g0, s_stat0, s_q1, s_g1, s_stat1) &&
-               step(s_q1, s_g1, s_stat1, s_q0, s_g0, s_stat0)) {
-        }
+        auto all = [&](auto low) GSD_INLINE {
+            while (step(low, s_q0, s_g0, s_stat0, s_q1, s_g1, s_stat1) &&
+                   step(low, s_q1, s_g1, s_stat1, s_q0, s_g0, s_stat0)) {
+            }
+        };
+        if (!kFew && __builtin_expect(keys <= kFewTerms, 0))
+            all(std::true_type{});
+        else
+            all(std::integral_constant<bool, kFew>{});
     }
     if (!valid) return;  // their gradients are written as 0 with delta
     const float fk = a.scale / (ds_scale * __builtin_ldexpf(1.0f, (int)T::kGradShift));
@@ -642,7 +654,8 @@ __global__ __launch_bounds__(kThreads, 2) void dkdv_pair_kernel(GradArgs g) {
 
     // with a mask, the block's keys are the next of the list
     const int at_key = (int)block * kPairHeld + (wave >> 1) * 32 + (lane & 31);
-    const bool valid = at_key < (a.list ? a.counts[b] : admitted_keys(a, b));
+    const int keys = a.list ? a.counts[b] : admitted_keys(a, b);
+    const bool valid = at_key < keys;
     const bool busy = ballot(valid) != 0;  // else a wave only loads and waits
     const int64_t key = a.list && valid ? a.list[(int64_t)b * a.keys + at_key] : at_key;
     f32x16 acc[DC / 32];
@@ -677,8 +690,9 @@ __global__ __launch_bounds__(kThreads, 2) void dkdv_pair_kernel(GradArgs g) {
         ds_scale = key_scale<T>(g, bh, v) * __builtin_ldexpf(1.0f, -(int)T::kGradShift);
         dma_wait();
         __syncthreads();
-        auto step = [&](const char* tile_q, const char* tile_g, const float* stat, char* next_q,
-                        char* next_g, float* next_stat) -> bool {
+        auto step = [&](auto low, const char* tile_q, const char* tile_g, const float* stat,
+                        char* next_q, char* next_g, float* next_stat) GSD_INLINE -> bool {
+            constexpr bool kLow = decltype(low)::value;
             const bool more = ++t < end;
             if (more) {
                 rq.next();
@@ -717,7 +731,7 @@ __global__ __launch_bounds__(kThreads, 2) void dkdv_pair_kernel(GradArgs g) {
                         const int j = 4 * i4 + i;
                         s[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j], a.scale_log2, of[i]));
                         dp[j] = s[j] * (dp[j] * ds_scale);
-                        if constexpr (kFew) dp[j] = formed(dp[j]);
+                        if constexpr (kLow) dp[j] = formed(dp[j]);
                     }
                 }
                 vec8 keep[2], keep_low[2];
@@ -726,7 +740,7 @@ __global__ __launch_bounds__(kThreads, 2) void dkdv_pair_kernel(GradArgs g) {
                     const vec8 p = pack<T>(s, j), ds = pack<T>(dp, j);
                     keep[j] = role ? ds : p;
                     s_pass[wave][j][lane] = __builtin_bit_cast(u32x4, role ? p : ds);
-                    if constexpr (kFew) {
+                    if constexpr (kLow) {
                         const vec8 p_low = pack_low<T>(s, j), ds_low = pack_low<T>(dp, j);
                         keep_low[j] = role ? ds_low : p_low;
                         pass_low[j] = __builtin_bit_cast(u32x4, role ? p_low : ds_low);
@@ -739,9 +753,9 @@ __global__ __launch_bounds__(kThreads, 2) void dkdv_pair_kernel(GradArgs g) {
                     for (int db = 0; db < DC / 32; ++db) {
                         const vec8 with = read_columns<T, DT>(mine + r0 * DT * 2, 16 * j, db);
                         acc[db] = T::mma(with, keep[j], acc[db]);
-                        if constexpr (kFew) acc[db] = T::mma(with, keep_low[j], acc[db]);
+                        if constexpr (kLow) acc[db] = T::mma(with, keep_low[j], acc[db]);
                     }
-                if constexpr (!kFew) pace<DC / 16, 2, 1, 3>();
+                if constexpr (!kLow) pace<DC / 16, 2, 1, 3>();
             }
             __syncthreads();
             auto add_passed = [&] {
@@ -756,7 +770,7 @@ __global__ __launch_bounds__(kThreads, 2) void dkdv_pair_kernel(GradArgs g) {
                 pace<DC / 16, 2, 1, 3>();
             };
             if (busy) add_passed();
-            if constexpr (kFew) {
+            if constexpr (kLow) {
                 // in the same place: with one more two work-groups would not fit a CU
                 __syncthreads();
                 if (busy)
@@ -771,9 +785,15 @@ __global__ __launch_bounds__(kThreads, 2) void dkdv_pair_kernel(GradArgs g) {
             }
             return more;
         };
-        while (step(s_q0, s_g0, s_stat0, s_q1, s_g1, s_stat1) &&
-               step(s_q1, s_g1, s_stat1, s_q0, s_g0, s_stat0)) {
-        }
+        auto all = [&](auto low) GSD_INLINE {
+            while (step(low, s_q0, s_g0, s_stat0, s_q1, s_g1, s_stat1) &&
+                   step(low, s_q1, s_g1, s_stat1, s_q0, s_g0, s_stat0)) {
+            }
+        };
+        if (!kFew && __builtin_expect(keys <= kFewTerms, 0))
+            all(std::true_type{});
+        else
+            all(std::integral_constant<bool, kFew>{});
     }
     if (!valid) return;
     const float f = role ? a.scale / (ds_scale * __builtin_ldexpf(1.0f, (int)T::kGradShift))

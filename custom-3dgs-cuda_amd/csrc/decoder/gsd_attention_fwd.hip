@@ -75,11 +75,13 @@ __global__ __launch_bounds__(kThreads, 2) void attention_kernel(AttnArgs a) {
     float m = -__builtin_inff(), off = T::kShift, sum = 0.0f;
 
     // one tile from its buffers, the next one's loads into the others; false
-    // after the last
-    auto step = [&](const char* tile_k, const char* tile_v, char* next_k, char* next_v) -> bool {
+    // after the last.  few: the only tile, where p's rounding is made up for
+    auto step = [&](auto few, const char* tile_k, const char* tile_v, char* next_k,
+                    char* next_v) GSD_INLINE -> bool {
+        constexpr bool kFew = decltype(few)::value;
         const int left = walk.left();
         walk.next();
-        const bool more = walk.more();
+        const bool more = !kFew && walk.more();
         if (more) {
             walk.look_ahead();
             keys.fetch(walk, next_k, next_v);
@@ -138,8 +140,12 @@ __global__ __launch_bounds__(kThreads, 2) void attention_kernel(AttnArgs a) {
                     // term, in the mean below the rounding of o itself
                     const vec8 p = pack<T>(s[h], k);
 #pragma unroll
-                    for (int db = 0; db < DC / 32; ++db)
-                        o[db] = T::mma(read_columns<T, DT>(tile_v, 32 * h + 16 * k, db), p, o[db]);
+                    for (int db = 0; db < DC / 32; ++db) {
+                        const vec8 vt = read_columns<T, DT>(tile_v, 32 * h + 16 * k, db);
+                        o[db] = T::mma(vt, p, o[db]);
+                        if constexpr (kFew)
+                            o[db] = T::mma(vt, pack_low<T>(s[h], k), o[db]);
+                    }
                 }
             }
         }
@@ -152,8 +158,12 @@ __global__ __launch_bounds__(kThreads, 2) void attention_kernel(AttnArgs a) {
     if (walk.more()) {
         dma_wait();
         __syncthreads();
-        while (step(s_k0, s_v0, s_k1, s_v1) && step(s_k1, s_v1, s_k0, s_v0)) {
-        }
+        if (__builtin_expect(walk.n <= kFewTerms, 0))
+            step(std::true_type{}, s_k0, s_v0, s_k1, s_v1);
+        else
+            while (step(std::false_type{}, s_k0, s_v0, s_k1, s_v1) &&
+                   step(std::false_type{}, s_k1, s_v1, s_k0, s_v0)) {
+            }
     }
     sum += other_half(sum);
     const float inv = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
@@ -325,6 +335,14 @@ __global__ __launch_bounds__(kThreads) void attention_few_kernel(AttnArgs a) {
             for (int db = 0; db < DT / 32; ++db)
                 o[db] = T::mma(read_columns<T, DT>(tile_v, 16 * k, db), p, o[db]);
         }
+        if (n <= kFewTerms)
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const vec8 p = pack_low<T>(s, k);
+#pragma unroll
+                for (int db = 0; db < DT / 32; ++db)
+                    o[db] = T::mma(read_columns<T, DT>(tile_v, 16 * k, db), p, o[db]);
+            }
     }
     sum += other_half(sum);
 
