@@ -50,6 +50,9 @@ Tensor dense_last(const Tensor& t) {
     return t.size(-1) <= 1 || t.stride(-1) == 1 ? t : t.contiguous();
 }
 
+// The stride of a dimension as the kernels step over it: over one element, never.
+int64_t step(const Tensor& t, int64_t d) { return t.size(d) > 1 ? t.stride(d) : 0; }
+
 // The attention kernels reach a tile's rows by offsets from its first: keys at
 // strides in [0, GSD_MAX_ATTENTION_STRIDE] or less, queries (in the backward) so that 65
 // of them and a group's heads span at most 2^30 elements.
@@ -61,13 +64,13 @@ Tensor near_keys(const Tensor& t, bool mask) {
         return stride >= 0 && stride <= GSD_MAX_ATTENTION_STRIDE &&
                !(mask && t.size(1) > 0 && stride >= span / t.size(1));
     };
-    if (fits(t.stride(1))) return dense_last(t);
+    if (fits(step(t, 1))) return dense_last(t);
     if (fits(t.size(2) * t.size(3))) return t.contiguous();
     return t.transpose(1, 2).contiguous().transpose(1, 2);  // head by head
 }
 Tensor near_queries(const Tensor& t, int64_t group) {
     const int64_t most = INT64_C(1) << 30;
-    const int64_t l = t.stride(1), h = t.stride(2);
+    const int64_t l = step(t, 1), h = step(t, 2);
     const bool ok = l >= 0 && h >= 0 && l < most / 65 && h < most / group &&
                     65 * l + group * h + t.size(3) <= most;
     return ok ? dense_last(t) : t.contiguous();
@@ -303,17 +306,17 @@ gsd_attention attention_args(const Tensor& q, const Tensor& k, const Tensor& v,
     a.kv_heads = k.size(2);
     a.dim = q.size(3);
     a.q = ptr(q);
-    a.q_stride_b = q.stride(0);
-    a.q_stride_l = q.stride(1);
-    a.q_stride_h = q.stride(2);
+    a.q_stride_b = step(q, 0);
+    a.q_stride_l = step(q, 1);
+    a.q_stride_h = step(q, 2);
     a.k = ptr(k);
-    a.k_stride_b = k.stride(0);
-    a.k_stride_l = k.stride(1);
-    a.k_stride_h = k.stride(2);
+    a.k_stride_b = step(k, 0);
+    a.k_stride_l = step(k, 1);
+    a.k_stride_h = step(k, 2);
     a.v = ptr(v);
-    a.v_stride_b = v.stride(0);
-    a.v_stride_l = v.stride(1);
-    a.v_stride_h = v.stride(2);
+    a.v_stride_b = step(v, 0);
+    a.v_stride_l = step(v, 1);
+    a.v_stride_h = step(v, 2);
     if (lengths.has_value()) {
         TORCH_CHECK(lengths->is_cuda() && lengths->device() == q.device() &&
                         lengths->scalar_type() == torch::kInt32 && lengths->dim() == 1 &&
@@ -397,9 +400,9 @@ std::tuple<Tensor, Tensor, Tensor> cross_attention_backward(
     dv = want_dkv ? torch::empty(v.sizes(), v.options()) : torch::empty({0}, q.options());
     gsd_attention_grad g{};
     g.d_o = ptr(grad);
-    g.do_stride_b = grad.stride(0);
-    g.do_stride_l = grad.stride(1);
-    g.do_stride_h = grad.stride(2);
+    g.do_stride_b = step(grad, 0);
+    g.do_stride_l = step(grad, 1);
+    g.do_stride_h = step(grad, 2);
     g.dq = ptr(dq);
     g.dk = ptr(dk);
     g.dv = ptr(dv);
