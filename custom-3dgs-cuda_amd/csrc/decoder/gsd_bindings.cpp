@@ -427,17 +427,19 @@ bool wants_grad(std::initializer_list<Tensor> inputs) {
     return false;
 }
 
-// The gradients are formed by kernels that record nothing: differentiating them
-// again raises, as it does through a once-differentiable Python function.
-tensor_list once(tensor_list out, const tensor_list& grads, const char* what) {
-    bool again = false;
-    for (const Tensor& g : grads) again = again || (g.defined() && g.requires_grad());
-    if (!at::GradMode::is_enabled() || !again) return out;
+// The gradients are formed by kernels that record nothing: a gradient that depends on
+// something that requires one, the incoming gradients or an input (where a constant
+// comes in, as sum()'s, that input alone), raises when it is differentiated again.
+Tensor once(const Tensor& t, bool depends, const char* what) {
+    if (!t.defined() || !depends || !at::GradMode::is_enabled()) return t;
     auto error = std::make_shared<torch::autograd::DelayedError>(
         std::string(what) + " is differentiable once", 1);
-    for (Tensor& t : out)
-        if (t.defined()) t = (*error)({t.detach().set_requires_grad(true)})[0];
-    return out;
+    return (*error)({t.detach().set_requires_grad(true)})[0];
+}
+bool any_requires_grad(const tensor_list& list) {
+    for (const Tensor& t : list)
+        if (t.defined() && t.requires_grad()) return true;
+    return false;
 }
 
 struct RotaryFunction : torch::autograd::Function<RotaryFunction> {
@@ -458,7 +460,8 @@ struct RotaryFunction : torch::autograd::Function<RotaryFunction> {
                                  ctx->saved_data["sections"].toIntVector(),
                                  ctx->saved_data["interleaved"].toBool(), true);
         }
-        return once(std::move(out), grads, "rotary_axes");
+        out[0] = once(out[0], any_requires_grad(grads), "rotary_axes");  // linear in x
+        return out;
     }
 };
 
@@ -477,6 +480,7 @@ struct NormFunction : torch::autograd::Function<NormFunction> {
         auto [y, h, rstd] = rms_norm_residual(x, residual, weight, eps, true);
         ctx->save_for_backward({h, rstd, weight});
         ctx->saved_data["residual"] = residual.has_value();
+        ctx->saved_data["of_h"] = any_requires_grad({x, or_undefined(residual)});
         ctx->set_materialize_grads(false);
         return {y, h};
     }
@@ -487,12 +491,17 @@ struct NormFunction : torch::autograd::Function<NormFunction> {
         if (!grads[0].defined()) {
             out[0] = grads[1];
         } else {
-            at::AutoGradMode off(false);
-            std::tie(out[0], out[2]) =
-                rms_norm_residual_backward(saved[0], saved[1], saved[2], grads[0], opt(grads[1]));
+            {
+                at::AutoGradMode off(false);
+                std::tie(out[0], out[2]) = rms_norm_residual_backward(saved[0], saved[1], saved[2],
+                                                                      grads[0], opt(grads[1]));
+            }
+            const bool of_h = ctx->saved_data["of_h"].toBool() || any_requires_grad(grads);
+            out[0] = once(out[0], of_h || saved[2].requires_grad(), "rms_norm_residual");
+            out[2] = once(out[2], of_h, "rms_norm_residual");
         }
         if (residual) out[1] = out[0];
-        return once(std::move(out), grads, "rms_norm_residual");
+        return out;
     }
 };
 
@@ -529,7 +538,11 @@ struct AttentionFunction : torch::autograd::Function<AttentionFunction> {
             if (want_k) out[1] = dk;
             if (want_v) out[2] = dv;
         }
-        return once(std::move(out), grads, "cross_attention");
+        const bool of_p = any_requires_grad({grads[0], s[0], s[1]});
+        for (int i = 0; i < 2; ++i)
+            out[i] = once(out[i], of_p || s[2].requires_grad(), "cross_attention");
+        out[2] = once(out[2], of_p, "cross_attention");
+        return out;
     }
 };
 
