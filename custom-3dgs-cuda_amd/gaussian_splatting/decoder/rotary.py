@@ -32,8 +32,8 @@ def rotary_axes(x: t.Tensor, positions: t.Tensor, inv_freq: t.Tensor, sections: 
 
     Returns:
         (B, L, H, D) contiguous; channels from 2 P on are x's.  Differentiable in x;
-        positions and inv_freq are data.
+        positions and inv_freq are data, and raise where a gradient would be wanted.
     """
-    if positions.requires_grad or inv_freq.requires_grad:
+    if t.is_grad_enabled() and (positions.requires_grad or inv_freq.requires_grad):
         raise ValueError("rotary_axes forms no gradient for positions or inv_freq: detach them")
     return module().decoder_rotary(x, positions, inv_freq, list(sections), interleaved)
