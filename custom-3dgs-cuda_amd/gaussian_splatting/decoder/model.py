@@ -54,7 +54,7 @@ class DecoderBlock(nn.Module):
         B, L, _ = x.shape
         y, residual = rms_norm_residual(x, residual, self.norm_attention)
         q = self.to_q(y).view(B, L, self.heads, self.head_dim)
-        kv = self.to_kv(tokens).view(B, -1, 2, self.kv_heads, self.head_dim)
+        kv = self.to_kv(tokens).view(B, tokens.shape[1], 2, self.kv_heads, self.head_dim)
         q = rotary_axes(q, query_pos, inv_freq, sections)
         k = rotary_axes(kv[:, :, 0], token_pos, inv_freq, sections)
         o = cross_attention(q, k, kv[:, :, 1], key_lengths=key_lengths, key_mask=key_mask)
@@ -66,7 +66,7 @@ class DecoderBlock(nn.Module):
         weight, weight_scale = eight_bit
         h = t._scaled_mm(y8.flatten(0, -2), weight.t(), scale_a=scale.reshape(-1, 1),
                          scale_b=weight_scale.reshape(1, -1), out_dtype=o.dtype)
-        return self.down(nn.functional.gelu(h.view(B, L, -1))), residual
+        return self.down(nn.functional.gelu(h.view(B, L, h.shape[1]))), residual
 
 
 class GaussianDecoder(nn.Module):
