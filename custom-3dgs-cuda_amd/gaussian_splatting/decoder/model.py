@@ -47,9 +47,30 @@ class DecoderBlock(nn.Module):
         self.out = make(heads * head_dim, width)
         self.up = make(width, 4 * width)
         self.down = make(4 * width, width)
+        self._eight_bit = None
+
+    def eight_bit_weight(self) -> tuple[t.Tensor, t.Tensor]:
+        """(codes, a scale per output) of ``up``'s weight, formed when first asked for and again
+        whenever the weight has changed: in place (its version says so), replaced, moved or
+        converted, or, with whatever wrote to it, after a forward with gradients."""
+        w = self.up.weight
+        version = None if w.is_inference() else w._version
+        if self._eight_bit is None or self._eight_bit[0] is not w or self._eight_bit[1] != version:
+            values = w.detach().float()
+            scale = values.abs().amax(1).clamp(min=1e-12) / 448.0
+            codes = (values / scale[:, None]).to(t.float8_e4m3fn)
+            self._eight_bit = (w, version, codes, scale)
+        return self._eight_bit[2:]
+
+    def forget_eight_bit_weight(self) -> None:
+        self._eight_bit = None
+
+    def _apply(self, *args, **kwargs):  # to(), half(), ...
+        self.forget_eight_bit_weight()
+        return super()._apply(*args, **kwargs)
 
     def forward(self, x, residual, tokens, query_pos, token_pos, inv_freq, sections, key_lengths,
-                key_mask, eight_bit=None):
+                key_mask, eight_bit=False):
         """(x, residual) after the block: x is still to be added to the residual stream."""
         B, L, _ = x.shape
         y, residual = rms_norm_residual(x, residual, self.norm_attention)
@@ -59,11 +80,11 @@ class DecoderBlock(nn.Module):
         k = rotary_axes(kv[:, :, 0], token_pos, inv_freq, sections)
         o = cross_attention(q, k, kv[:, :, 1], key_lengths=key_lengths, key_mask=key_mask)
         o = self.out(o.flatten(-2))
-        if eight_bit is None:
+        if not eight_bit:
             y, residual = rms_norm_residual(o, residual, self.norm_network)
             return self.down(nn.functional.gelu(self.up(y))), residual
         y8, scale, residual = rms_norm_residual_fp8(o, residual, self.norm_network)
-        weight, weight_scale = eight_bit
+        weight, weight_scale = self.eight_bit_weight()
         h = t._scaled_mm(y8.flatten(0, -2), weight.t(), scale_a=scale.reshape(-1, 1),
                          scale_b=weight_scale.reshape(1, -1), out_dtype=o.dtype)
         return self.down(nn.functional.gelu(h.view(B, L, h.shape[1]))), residual
@@ -93,16 +114,19 @@ class GaussianDecoder(nn.Module):
         self.head = nn.Linear(width, ATTRIBUTES)  # attributes are 32-bit
         nn.init.normal_(self.head.weight, std=0.02)
         nn.init.zeros_(self.head.bias)
-        self._eight_bit = None
+        self._serve_eight_bits = False
 
-    def serve_in_eight_bits(self) -> None:
+    def serve_in_eight_bits(self, on: bool = True) -> None:
         """From here on, without gradients, the blocks' first network layer takes its input
-        from ``rms_norm_residual_fp8`` and its weights in 8 bits with a scale per output."""
-        self._eight_bit = []
+        from ``rms_norm_residual_fp8`` and its weights in 8 bits with a scale per output; with
+        ``on`` false, no longer.  The 8-bit weights are no part of the state: they follow the
+        weights through further training, loading and moving.  Only a write through ``.data``
+        without a forward with gradients before the next answer goes unseen: call this again."""
+        self._serve_eight_bits = on
         for block in self.blocks:
-            w = block.up.weight.detach().float()
-            scale = w.abs().amax(1).clamp(min=1e-12) / 448.0
-            self._eight_bit.append(((w / scale[:, None]).to(t.float8_e4m3fn), scale))
+            block.forget_eight_bit_weight()
+            if on:
+                block.eight_bit_weight()
 
     def forward(self, tokens: t.Tensor, token_pos: t.Tensor, query_pos: t.Tensor,
                 key_lengths: t.Tensor | None = None,
@@ -116,11 +140,12 @@ class GaussianDecoder(nn.Module):
         B, L = tokens.shape[0], query_pos.shape[-2]
         x = self.query.expand(B, L, -1).contiguous()
         residual = None
-        eight = self._eight_bit if not t.is_grad_enabled() else None
-        for i, block in enumerate(self.blocks):
+        eight = self._serve_eight_bits and not t.is_grad_enabled()
+        for block in self.blocks:
+            if t.is_grad_enabled():  # training may go on, by any means of writing the weights
+                block.forget_eight_bit_weight()
             x, residual = block(x, residual, tokens, query_pos, token_pos, self.inv_freq,
-                                self.sections, key_lengths, key_mask,
-                                None if eight is None else eight[i])
+                                self.sections, key_lengths, key_mask, eight)
         y, _ = rms_norm_residual(x, residual, self.norm_head)
         return self.head(y.float())
 
