@@ -85,8 +85,10 @@ class DecoderBlock(nn.Module):
             return self.down(nn.functional.gelu(self.up(y))), residual
         y8, scale, residual = rms_norm_residual_fp8(o, residual, self.norm_network)
         weight, weight_scale = self.eight_bit_weight()
+        # the library's product with a scale per row answers in bf16 only, whose 2^-9 is small
+        # beside the codes' 2^-4
         h = t._scaled_mm(y8.flatten(0, -2), weight.t(), scale_a=scale.reshape(-1, 1),
-                         scale_b=weight_scale.reshape(1, -1), out_dtype=o.dtype)
+                         scale_b=weight_scale.reshape(1, -1), out_dtype=t.bfloat16).to(o.dtype)
         return self.down(nn.functional.gelu(h.view(B, L, h.shape[1]))), residual
 
 
