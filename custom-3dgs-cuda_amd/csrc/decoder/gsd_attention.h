@@ -268,8 +268,10 @@ __device__ __forceinline__ u32x4 buffer_at(const char* base) {
 // and so for memory once per tile.  dma_wait() waits for those of the wave; a
 // barrier behind it makes the work-group's visible.  The first s_nop covers the
 // five states between a scalar register's write by a vector instruction and its
-// use by a memory one, the others the one after a write of m0.  kStream: data that is
-// read once and not kept in the caches.
+// use by a memory one, the others the one after a write of m0.  m0 is reserved: the
+// compiler does not keep it over assembly that names it as changed (it warns there), so
+// these kernels hold no other instruction that uses it.  kStream: data that is read once
+// and not kept in the caches.
 #define GSD_DMA16_X4(kind)                                                                   \
     asm volatile(                                                                            \
         "s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %5, 0 offen" kind " lds\n\t"   \
