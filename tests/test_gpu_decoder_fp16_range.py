@@ -148,3 +148,14 @@ def test_a_row_whose_gradient_is_not_finite_leaves_the_others_dq(device, bad, na
         rest[0, 7, 1] = False
         assert got[~rest].isnan().all()
         assert t.equal(got[rest], clean[rest])
+
+
+@pytest.mark.parametrize("size", [1e-6, 2.0 ** 12])
+@pytest.mark.parametrize("L,S,D", [(100, 300, 64), (40, 1200, 128)])
+def test_gradients_of_a_mean_and_of_a_scaled_loss(device, size, L, S, D):
+    """do of 1e-6, itself below the type's normal range, and of 2^12."""
+    print(f"[gpu] fp16 range, do of {size} {(L, S, D)}", flush=True)
+    randn = _randn(device, L)
+    q, k, v = randn(1, L, 2, D).half(), randn(1, S, 2, D).half(), randn(1, S, 2, D).half()
+    do = (size * randn(1, L, 2, D)).half()
+    _assert_rows(_gradients(q, k, v, do), _exact(q, k, v, do), 1.5, (size, L, S, D))
