@@ -158,7 +158,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_kernel(AttnArgs a) {
     if (walk.more()) {
         dma_wait();
         __syncthreads();
-        if (__builtin_expect(walk.n <= kFewTerms, 0))
+        if (walk.n <= kFewTerms)
             step(std::true_type{}, s_k0, s_v0, s_k1, s_v1);
         else
             while (step(std::false_type{}, s_k0, s_v0, s_k1, s_v1) &&
