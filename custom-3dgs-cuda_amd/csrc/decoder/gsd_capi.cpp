@@ -40,7 +40,10 @@ inline size_t align_up(size_t x) { return (x + 255) / 256 * 256; }
 
 constexpr int64_t kMaxCount = INT64_C(1) << 31;  // of any one dimension
 constexpr int64_t kMaxListSpan = (INT64_C(1) << 30) - 1024;  // elements
-constexpr int64_t kMaxGroups = INT64_C(2147483647);
+// a launch holds fewer than 2^32 work-items: work-groups of 256, and of 1024 (one per batch)
+// where a mask is listed
+constexpr int64_t kMaxGroups = (INT64_C(1) << 24) - 1;
+constexpr int64_t kMaxListed = (INT64_C(1) << 22) - 1;
 
 inline bool dtype_ok(int d) { return d == GSD_F32 || d == GSD_BF16 || d == GSD_F16; }
 inline int dtype_size(int d) { return d == GSD_F32 ? 4 : 2; }
@@ -93,6 +96,7 @@ int check_attention(const gsd_attention* a) {
     GSD_REQUIRE(!a->key_mask || (a->keys * a->k_stride_l < kMaxListSpan &&
                                  a->keys * a->v_stride_l < kMaxListSpan),
                 "with a mask, keys x their stride must lie below 2^30");
+    GSD_REQUIRE(!a->key_mask || a->batch <= kMaxListed, "with a mask, batch must lie below 2^22");
     GSD_REQUIRE(product_fits(a->batch, a->queries, a->heads * a->dim * 4) &&
                     product_fits(a->batch, a->keys, a->kv_heads * a->dim * 4),
                 "the tensors are too large");
@@ -203,7 +207,7 @@ int gsd_rotary_axes(const gsd_rotary* a, void* stream) {
                 (long long)(2 * pairs), (long long)a->dim);
     // a thread takes four values at least, in 32-bit counts
     const __int128 n = (__int128)a->batch * a->length * a->heads * a->dim;
-    GSD_REQUIRE((__int128)a->batch * a->length * a->heads * (a->dim / 4 + 2) < kMaxCount * 2,
+    GSD_REQUIRE((__int128)a->batch * a->length * a->heads * (a->dim / 4 + 2) <= 256 * kMaxGroups,
                 "the tensor is too large");
     if (n == 0) return GSR_OK;
     GSD_REQUIRE(a->x && a->y && (pairs == 0 || (a->positions && a->inv_freq)), "null pointer");

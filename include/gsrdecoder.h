@@ -6,13 +6,15 @@
  *
  * Plain pointers and sizes only; tensor arguments are DEVICE pointers, strides
  * count elements and may be zero (a broadcast) or, where not said otherwise,
- * negative; the last dimension is contiguous everywhere.  `stream` is a hipStream_t (NULL = the null
- * stream); all work is enqueued on it, nothing waits, and nothing allocates.
+ * negative; the last dimension is contiguous everywhere.  `stream` is a
+ * hipStream_t (NULL = the null stream); all work is enqueued on it, nothing
+ * waits, and nothing allocates.
  * Pointers need only their elements' own alignment.
  *
  * Every entry point returns GSR_OK or one of gsraster.h's error codes;
  * gsd_last_error() gives the calling thread's message for the last failure.
- * Outputs are contiguous and fully written by the call.
+ * Outputs are contiguous, fully written by the call and overlap no input.  Calls
+ * whose launches would hold 2^32 work-items are refused.
  */
 #ifndef GSRDECODER_H
 #define GSRDECODER_H
