@@ -13,8 +13,10 @@
 // blocks with atomics, whose order changes results, or through memory.
 //
 // As in the forward, matrix products and vector instructions bound them.  4096 x
-// 32400, 16 heads of 128 in groups of 4: dk and dv 2.01 to 2.07 ms by card (1.05 to
-// 1.08 PFLOP/s), dq 1.34 to 1.38 ms (1.18 to 1.22), delta 10 us (5 TB/s).
+// 32400, 16 heads of 128 in groups of 4: dk and dv 2.00 to 2.09 ms by card (1.04 to
+// 1.09 PFLOP/s; 0.52 of a SIMD's cycles with a matrix instruction, 0.35 with a vector
+// one, 0.08 with both), dq 1.30 to 1.38 ms (1.18 to 1.25; 0.65, 0.33 and 0.10), delta 11
+// us (5 TB/s).
 #include "gsd_attention.h"
 
 namespace gsd {

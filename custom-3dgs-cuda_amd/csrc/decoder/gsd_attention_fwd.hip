@@ -7,12 +7,14 @@
 // p^T takes p from those registers.  Keys and values pass through LDS in tiles
 // of 64, two buffers, the next tile's loads in flight during the products.
 //
-// Matrix products and the vector instructions around the exponentials bound it:
-// a wave does one or the other, so two waves on a SIMD (heads of 128, whose sums
-// and q take their registers) or four (64) do them side by side.  4096 x 32400, 16
-// heads of 128: 0.97 ms, 1.12 PFLOP/s (a large library product reaches 1.34); 4096 x
-// 16200, 16 heads of 64, where an exponential goes with half the products: 0.32 ms,
-// 0.84 PFLOP/s.
+// Matrix products and the vector instructions around the exponentials bound it.  A
+// wave does one or the other, so two waves on a SIMD (heads of 128, whose sums and q
+// take their registers) or four (64) share it.  Counters give, of a SIMD's cycles, 0.59
+// with a matrix instruction, 0.49 with a vector one and 0.21 with both at once for heads
+// of 128, at the 1.8 GHz that the card then runs at; for heads of 64, where an exponential
+// goes with half the products, 0.43, 0.65 and 0.24.  4096 x 32400, 16 heads of 128: 0.96
+// to 1.01 ms by card, 1.08 to 1.14 PFLOP/s (a large library product reaches 1.34); 4096 x
+// 16200, 16 heads of 64: 0.31 ms, 0.87 PFLOP/s.
 //
 // Where the rows make too few work-groups, the keys are split into parts whose
 // normalised sums and log-sums a second kernel joins.
