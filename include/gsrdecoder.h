@@ -130,7 +130,8 @@ int gsd_rms_norm_backward(int dtype, int64_t rows, int64_t width, const void* h,
  * is what the rounding of o left out, rounded to the type in its turn: with it the
  * backward forms sum do o from 32-bit values, which matters where a query has few
  * keys (a few dozen).  Sums and statistics are held in 32 bits; p is rounded to the
- * type for its product with v. */
+ * type for its product with v, and with up to 64 valid keys what that leaves out is
+ * multiplied too. */
 typedef struct gsd_attention {
     int dtype;
     int64_t batch, queries, keys, heads, kv_heads, dim;
