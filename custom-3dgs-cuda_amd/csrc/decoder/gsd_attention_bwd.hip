@@ -78,7 +78,7 @@ __device__ __forceinline__ void zero_keys(const GradArgs& g, uint32_t group) {
     store_any(g.dv + 16 * id, u32x4{0, 0, 0, 0});
 }
 
-// The maximum over a work-group, in its first thread.
+// The maximum over a work-group.
 __device__ __forceinline__ float group_max(float v, float (&part)[kWaves]) {
     v = wave_max(v);
     if (lane_id() == 0) part[threadIdx.x / kWave] = v;
